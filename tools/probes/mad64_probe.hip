@@ -1,5 +1,5 @@
 // probe: what does v_mad_u64_u32 (Philox's 32 x 32 -> 64 product in one instruction) cost next to v_mul_lo_u32 + v_mul_hi_u32 on gfx950?
-//   hipcc --offload-arch=gfx950 -O3 -o /tmp/mad64_probe tools/probes/mad64_probe.hip && /tmp/mad64_probe
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o /tmp/mad64_probe tools/probes/mad64_probe.hip && /tmp/mad64_probe
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #define CK(x) do { hipError_t e_ = (x); if (e_ != hipSuccess) { printf("HIP error %s at %d\n", hipGetErrorString(e_), __LINE__); return 1; } } while (0)

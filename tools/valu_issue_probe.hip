@@ -11,7 +11,7 @@
 // Also run with a partial EXEC mask (lanes 0-31 only, lanes 0-15 only, every other lane): does the hardware skip the
 // idle half of a wave?  (It decides whether compacting walkers to the low lanes could pay.)
 //
-// Build + run (GPU box):  hipcc --offload-arch=gfx950 -O2 tools/valu_issue_probe.hip -o /tmp/valu_probe && /tmp/valu_probe
+// Build + run (GPU box):  hipcc --offload-arch=gfx950 -O2 -Xclang -target-feature -Xclang -packed-fp32-ops tools/valu_issue_probe.hip -o /tmp/valu_probe && /tmp/valu_probe
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -52,7 +52,6 @@ constexpr int UNROLL = 32;       // instructions per loop body (8 chains x 4)
 #define OP_EXP(i) "v_exp_f32 %" i ", %" i "\n"
 #define OP_CVT(i) "v_cvt_f32_u32 %" i ", %" i "\n"
 #define OP_FLOOR(i) "v_floor_f32 %" i ", %" i "\n"
-#define OP_PKFMA(i) "v_pk_fma_f32 %" i ", %" i ", %8, %9\n"       /* only valid on 64-bit operands: see kernel below */
 #define OP_DIVFIX(i) "v_div_fixup_f32 %" i ", %" i ", %8, %9\n"
 #define OP_FMAS(i) "v_fma_f32 %" i ", %" i ", %10, %9\n"          /* one SGPR operand */
 #define OP_MED3(i) "v_med3_f32 %" i ", %" i ", %8, %9\n"
@@ -81,13 +80,13 @@ constexpr int UNROLL = 32;       // instructions per loop body (8 chains x 4)
 
 enum {
     K_FMA, K_FMA_DEP, K_ADDF, K_MULF, K_MAXF, K_ADDU, K_AND, K_LSHL, K_MOV, K_MULLO, K_MULHI, K_MUL24, K_MAD24, K_CNDMASK, K_CMP,
-    K_RCP, K_SQRT, K_LOG, K_EXP, K_CVT, K_FLOOR, K_DIVFIX, K_FMAS, K_MED3, K_BFE, K_DPP, K_READFIRST, K_FMA64, K_PKFMA, K_DSREAD, K_CND64, K_CMP64, K_CMPCND, K_ADDCO, K_CMPU, K_MINF, K_SUBF, K_FMAC, K_MADF, K_XOR, K_LSHLADD, K_ADD3, K_CVTI, K_MULLIT, K_ADDK, K_CMPFMA, K_SALU, K_SAND64, K_P1, K_P2, K_P3, K_P4, K_P5, K_P6, K_P7, K_ADDS, K_MULS, K_FMACS, K_SUBS, K_ADDUS, K_FMA2S, K_MAXK, K_COUNT
+    K_RCP, K_SQRT, K_LOG, K_EXP, K_CVT, K_FLOOR, K_DIVFIX, K_FMAS, K_MED3, K_BFE, K_DPP, K_READFIRST, K_FMA64, K_DSREAD, K_CND64, K_CMP64, K_CMPCND, K_ADDCO, K_CMPU, K_MINF, K_SUBF, K_FMAC, K_MADF, K_XOR, K_LSHLADD, K_ADD3, K_CVTI, K_MULLIT, K_ADDK, K_CMPFMA, K_SALU, K_SAND64, K_P1, K_P2, K_P3, K_P4, K_P5, K_P6, K_P7, K_ADDS, K_MULS, K_FMACS, K_SUBS, K_ADDUS, K_FMA2S, K_MAXK, K_COUNT
 };
 static const char* kNames[K_COUNT] = {
     "v_fma_f32 (8 chains)", "v_fma_f32 (1 dependent chain)", "v_add_f32", "v_mul_f32", "v_max_f32", "v_add_u32", "v_and_b32", "v_lshlrev_b32",
     "v_mov_b32", "v_mul_lo_u32", "v_mul_hi_u32", "v_mul_u32_u24", "v_mad_u32_u24", "v_cndmask_b32", "v_cmp_lt_f32", "v_rcp_f32", "v_sqrt_f32",
     "v_log_f32", "v_exp_f32", "v_cvt_f32_u32", "v_floor_f32", "v_div_fixup_f32", "v_fma_f32 (SGPR operand)", "v_med3_f32", "v_bfe_u32",
-    "v_mov_b32_dpp quad_perm", "v_readfirstlane_b32", "v_fma_f64", "v_pk_fma_f32", "ds_read_b32 (conflict-free)",
+    "v_mov_b32_dpp quad_perm", "v_readfirstlane_b32", "v_fma_f64", "ds_read_b32 (conflict-free)",
     "v_cndmask_b32_e64 (s[20:21])", "v_cmp_lt_f32_e64 -> s[20:21]", "v_cmp vcc + v_cndmask vcc (per pair)", "v_add_co_u32 (vcc out)", "v_cmp_lt_u32 vcc",
     "v_min_f32", "v_sub_f32", "v_fmac_f32", "v_mul_legacy_f32", "v_xor_b32", "v_lshl_add_u32", "v_add3_u32", "v_cvt_i32_f32", "v_mul_f32 (32-bit literal)",
     "v_add_f32 (inline const)", "v_cmp + 3 v_fma (per 4)", "s_add_u32", "s_and_b64",
@@ -179,13 +178,6 @@ __global__ __launch_bounds__(256) void probe(unsigned long long* spans, float* s
                 asm volatile(".rept 4\n"
                              "v_fma_f64 %0, %0, %8, %9\n v_fma_f64 %1, %1, %8, %9\n v_fma_f64 %2, %2, %8, %9\n v_fma_f64 %3, %3, %8, %9\n"
                              "v_fma_f64 %4, %4, %8, %9\n v_fma_f64 %5, %5, %8, %9\n v_fma_f64 %6, %6, %8, %9\n v_fma_f64 %7, %7, %8, %9\n"
-                             ".endr\n"
-                             : "+v"(d0), "+v"(d1), "+v"(d2), "+v"(d3), "+v"(d4), "+v"(d5), "+v"(d6), "+v"(d7) : "v"(da), "v"(db));
-            } else if (KIND == K_PKFMA) {
-                // the 64-bit register pairs of the doubles serve as float2 operands
-                asm volatile(".rept 4\n"
-                             "v_pk_fma_f32 %0, %0, %8, %9\n v_pk_fma_f32 %1, %1, %8, %9\n v_pk_fma_f32 %2, %2, %8, %9\n v_pk_fma_f32 %3, %3, %8, %9\n"
-                             "v_pk_fma_f32 %4, %4, %8, %9\n v_pk_fma_f32 %5, %5, %8, %9\n v_pk_fma_f32 %6, %6, %8, %9\n v_pk_fma_f32 %7, %7, %8, %9\n"
                              ".endr\n"
                              : "+v"(d0), "+v"(d1), "+v"(d2), "+v"(d3), "+v"(d4), "+v"(d5), "+v"(d6), "+v"(d7) : "v"(da), "v"(db));
             } else if (KIND == K_DSREAD) {
@@ -293,7 +285,7 @@ int main() {
     }
     // wall-clock cross-check: the s_memtime rate, and the whole-chip rate of the saturated launch
     printf("\n== wall clock (HIP events) of the 8-blocks-per-CU launch ==\n");
-    for (int k : {(int)K_FMA, (int)K_ADDF, (int)K_ADDU, (int)K_MULLO, (int)K_RCP, (int)K_CNDMASK, (int)K_PKFMA}) {
+    for (int k : {(int)K_FMA, (int)K_ADDF, (int)K_ADDU, (int)K_MULLO, (int)K_RCP, (int)K_CNDMASK}) {
         float ms = 0;
         const Result r = run(k, cus * 8, ~0ull, &ms);
         const double wave_instr = instr * cus * 8 * 4;
