@@ -430,7 +430,7 @@ def main():
         st = hb.ctx.stats()                               # per-kernel HIP-event times of the LAST step (events on the ctx stream)
         if multi:
             t = torch.tensor([elapsed], dtype=torch.float64, device=dev)
-            dist.all_reduce(t, op=dist.ReduceOp.MAX)
+            pkg.dist.all_reduce(t, dist.ReduceOp.MAX)
             elapsed = float(t.item())
         samples_per_step_rank = W * H * spp
         value = W * H * job_iters * steps / elapsed / 1e6

@@ -33,6 +33,22 @@ def init_comm(ctx, group=None):
     return ctx
 
 
+def _host_only(t, group=None):
+    """does the backend that carries t's device take host memory only?  gloo accepts device tensors, but ranks that share one GPU have hung in it"""
+    config = dict(b.split(":") for b in str(dist.get_backend_config(group)).split(","))
+    return t.device.type != "cpu" and config.get(t.device.type) == "gloo"
+
+
+def all_reduce(t, op=dist.ReduceOp.SUM, group=None):
+    """torch.distributed's all-reduce of t, in place.  Over gloo a device tensor goes through host memory, with synchronous copies both ways."""
+    if not _host_only(t, group):
+        dist.all_reduce(t, op=op, group=group)
+        return t
+    host = t.cpu()
+    dist.all_reduce(host, op=op, group=group)
+    return t.copy_(host)
+
+
 def combine_means(accum, n_local, group=None, ctx=None, stream=None):
     """In place: accum <- global mean.  accum: [n_pixels, 3] fp32 running mean over this rank's
     n_local iterations.
@@ -40,7 +56,7 @@ def combine_means(accum, n_local, group=None, ctx=None, stream=None):
     ctx with a communicator (init_comm): the C-ABI collective, enqueued on `stream` (a raw HIP stream
     handle; None = the context's own stream) -- asynchronous, ordered with the renders on that stream.
     Otherwise: one torch.distributed all-reduce of the weighted sums, the count riding along as one
-    extra element (gloo on CPU tensors in the tests)."""
+    extra element (over gloo through host memory: all_reduce)."""
     if ctx is not None and getattr(ctx, "comm_nranks", 0) > 0:
         ctx.allreduce_accum(accum, n_local, stream)
         return accum
@@ -50,6 +66,6 @@ def combine_means(accum, n_local, group=None, ctx=None, stream=None):
     buf = torch.empty(flat.numel() + 1, dtype=torch.float32, device=accum.device)
     torch.mul(flat, float(n_local), out=buf[:-1])
     buf[-1] = float(n_local)
-    dist.all_reduce(buf, op=dist.ReduceOp.SUM, group=group)
+    all_reduce(buf, dist.ReduceOp.SUM, group)
     torch.div(buf[:-1], buf[-1], out=flat)
     return accum
