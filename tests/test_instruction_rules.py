@@ -101,3 +101,10 @@ def test_no_source_spells_out_packed_fp32():
 
 def test_no_code_object_holds_packed_fp32(instructions):
     assert not {o for o in instructions if PACKED_FP32.match(o)}
+
+
+def test_build_turns_the_packed_fp32_feature_off():
+    """the compiler's own vectorisers and combines may form packed fp32 from ordinary float code: the feature is off for every HIP source"""
+    import __graft_entry__ as ge
+    flags = " ".join(ge._load_build_module().COMMON)
+    assert "-Xclang -target-feature -Xclang -packed-fp32-ops" in flags

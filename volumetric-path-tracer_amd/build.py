@@ -26,7 +26,10 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # -fno-slp-vectorize: the SLP vectoriser turns pairs of fp32 operations into packed v_pk_* instructions -- the same issue cost as the two
 # scalar ones on gfx950 (profiles/r02_valu_issue_probe.txt) but operands in aligned VGPR pairs, constants included: the direct tracer needs
 # 133 registers without them and 158 with (profiles/r04_four_waves.txt); every kernel of the path is at least as fast without.
-COMMON = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function", "-Wno-unused-variable", "-fno-slp-vectorize"]
+# -packed-fp32-ops: some packed fp32 forms have given wrong results on these cards, and the SLP vectoriser is not the only pass that may form
+# them.  Times are equal with and without (1920x1080 dragon, 64 iterations: 4.65 ms per step either way).  The host pass does not know the feature and says so.
+PACKED_FP32_OFF = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+COMMON = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function", "-Wno-unused-variable", "-fno-slp-vectorize"] + PACKED_FP32_OFF
 STRICT = ["-ffp-contract=off", "-fno-fast-math"]
 VALUE_ONLY = ["-ffp-contract=off", "-fno-hip-fp32-correctly-rounded-divide-sqrt"]
 SOURCES = {
@@ -124,7 +127,7 @@ def build_cli(verbose=False):
     deps = [CLI_SRC, OUT, os.path.join(inc, "vpt_abi.h"), os.path.join(inc, "vpt_io.h")]
     if not _stale(CLI_OUT, deps):
         return CLI_OUT
-    cmd = [HIPCC, "-O2", "-std=c++17", "-x", "hip", "--offload-arch=gfx950", "-I", inc, CLI_SRC, "-o", CLI_OUT,
+    cmd = [HIPCC, "-O2", "-std=c++17", "-x", "hip", "--offload-arch=gfx950"] + PACKED_FP32_OFF + ["-I", inc, CLI_SRC, "-o", CLI_OUT,
            "-L", HERE, "-lvpt_hip", "-Wl,-rpath,$ORIGIN"]
     if verbose:
         print(" ".join(cmd), flush=True)
