@@ -2,7 +2,7 @@
 # Run on the GPU box: rocprofv3 kernel-trace stats + PMC passes of the bench command, summarised
 # into gpurun_out/<tag>_*.txt (copy the ones to keep into profiles/).
 #   tools/profile_bench.sh <tag> [bench args...]
-set -u
+set -eu -o pipefail      # a pass that fails or runs out of time ends the script: nothing more is started on the GPU
 TAG=${1:-prof}; shift || true
 ARGS=${@:---steps 2 --warmup 1 --no-cpu-baseline --no-other-configs --no-per-frame}
 REPO=$(cd "$(dirname "$0")/.." && pwd)
@@ -12,8 +12,8 @@ cd /tmp && export TMPDIR=/tmp
 run() {  # name, rocprof flags...
   local name=$1; shift
   rm -rf /tmp/rp_$name
-  rocprofv3 "$@" -d /tmp/rp_$name -o r -- python $REPO/bench.py $ARGS > $OUT/${TAG}_${name}.log 2>&1
-  find /tmp/rp_$name -name "*.db" | head -1
+  timeout -s KILL ${PASS_LIMIT:-150} rocprofv3 "$@" -d /tmp/rp_$name -o r -- python $REPO/bench.py $ARGS > $OUT/${TAG}_${name}.log 2>&1 || return
+  find /tmp/rp_$name -name "*.db" -print -quit
 }
 DB=$(run kt --kernel-trace --stats)
 # every summary names the commit it was taken at (COMMIT: passed in by the caller, the GPU box has no .git)
